@@ -20,17 +20,12 @@ I16, I32, I64, F64 = torch.int16, torch.int32, torch.int64, torch.float64
 ONE = 1 << 16
 
 
-_loaded = None
-
-
 def _ops():
-    """the engine's operators, imported once as a program does"""
-    global _loaded
-    if _loaded is None:
-        sys.path.insert(0, os.path.join(os.getcwd(), "exact-llm_amd"))
-        from exact_amd import ops
-        _loaded = ops
-    return _loaded
+    path = os.path.join(os.getcwd(), "exact-llm_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from exact_amd import ops
+    return ops
 
 
 # ----------------------------------------------------------------------------- the cases
