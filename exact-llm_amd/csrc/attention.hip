@@ -253,7 +253,7 @@ __global__ __launch_bounds__(ATT_THREADS) void k_attention(const int16_t* __rest
   mx = block_max64(mx, red);
   int64_t es = 0;
   for (int si = tid; si < S; si += blockDim.x) {
-    const int64_t e = lut_exp(expt, mx - sc[si]);
+    const int64_t e = lut_exp(expt, mx, sc[si]);
     sc[si] = e;
     es += e;
   }
@@ -544,7 +544,7 @@ __global__ __launch_bounds__(NT) void k_attention_qkv(const int64_t* __restrict_
   mx = block_max64_1(mx, red);
   int64_t es = 0;
   for (int si = tid; si < S; si += blockDim.x) {
-    const int64_t e = lut_exp(GT ? expt : texp, mx - sc[si]);
+    const int64_t e = lut_exp(GT ? expt : texp, mx, sc[si]);
     sc[si] = e;
     es += e;
   }
@@ -811,7 +811,7 @@ __global__ __launch_bounds__(NT) void k_attention_gqa(const int64_t* __restrict_
   for (int si = tid; si < S; si += NT) {
 #pragma unroll
     for (int hb = 0; hb < HB; ++hb) {
-      const int64_t e = lut_exp(expt, mx[hb] - sc[hb * Smax + si]);
+      const int64_t e = lut_exp(expt, mx[hb], sc[hb * Smax + si]);
       sc[hb * Smax + si] = e;
       es[hb] += e;
     }

@@ -193,7 +193,7 @@ __global__ __launch_bounds__(64 * HB) void k_dec_exp(const int64_t* __restrict__
 #pragma unroll
   for (int j = 0; j < EPT; ++j) {
     const int i = k0 + lane + 64 * j;
-    const int e = i <= p ? (int)lut_exp(expt, mx - x[j]) : 0;
+    const int e = i <= p ? (int)lut_exp(expt, mx, x[j]) : 0;
     el[row * Sp + i] = e;
     es += e;
   }

@@ -631,7 +631,7 @@ __device__ __forceinline__ void passes12_i64(const QK& c, const AttnLDS& L, cons
     scores_i64(c, 32 * t, hh, xx, ll, rterm, sqv, INV, sc);
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      if (valid(t, i)) e += lut_exp(Tg, mx - sc[i]);
+      if (valid(t, i)) e += lut_exp(Tg, mx, sc[i]);
   }
   e += __shfl_xor(e, 32, 64);
   if (c.half == 0) L.red_b[w * 32 + c.l32] = e;
@@ -660,7 +660,7 @@ __device__ __forceinline__ void produce_i64(const QK& c, const AttnLDS& L, const
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const bool ok = 32 * t + 8 * (i >> 2) + 4 * c.half + (i & 3) <= mypos;
-          p[i] = ok ? (int)floordiv_rcp(shl64(lut_exp(Tg, mx - sc[i]), 20), es, res) : 0;
+          p[i] = ok ? (int)floordiv_rcp(shl64(lut_exp(Tg, mx, sc[i]), 20), es, res) : 0;
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {

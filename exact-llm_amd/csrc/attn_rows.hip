@@ -83,7 +83,7 @@ __global__ __launch_bounds__(ROWS_WAVES * 64) void k_attention_rows(
   int64_t es = 0, e[NK];
 #pragma unroll
   for (int c = 0; c < NK; ++c) {
-    e[c] = 64 * c + lane < S ? lut_exp(expt, mx - x[c]) : 0;
+    e[c] = 64 * c + lane < S ? lut_exp(expt, mx, x[c]) : 0;
     es += e[c];
   }
   es = wave_sum64(es);

@@ -815,7 +815,7 @@ __global__ __launch_bounds__(512) void k_tree_short(const int16_t* __restrict__ 
           int64_t dot = 0;
           for (int j = 0; j < HD; ++j) dot += (256 * qp[j] + qp[HD + j] + 128) * (int)kq[(cbase + k) * HD + j];
           const int64_t x = shr64(dot * INV, 32 - W.shq[row0 + m0 + r] - sk[cbase + k]);
-          p = floordiv_pos(shl64(lut_exp_below(expt, xm[0][r], x), 20), xs[0][r]);
+          p = floordiv_pos(shl64(lut_exp(expt, xm[0][r], x), 20), xs[0][r]);
         }
         ps[tid] = p;
         __syncthreads();

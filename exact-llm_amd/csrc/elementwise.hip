@@ -282,10 +282,10 @@ __global__ void k_isoftmax(const int64_t* __restrict__ sc, const int32_t* __rest
   for (int i = threadIdx.x; i < nv; i += blockDim.x) mx = row[i] > mx ? row[i] : mx;
   mx = block_max64(mx, red);
   int64_t es = 0;
-  for (int i = threadIdx.x; i < nv; i += blockDim.x) es += lut_exp(T, mx - row[i]);
+  for (int i = threadIdx.x; i < nv; i += blockDim.x) es += lut_exp(T, mx, row[i]);
   es = block_sum64(es, red);
   for (int i = threadIdx.x; i < N; i += blockDim.x)
-    p[(int64_t)r * N + i] = i < nv ? floordiv_pos(shl64(lut_exp(T, mx - row[i]), 20), es) : 0;
+    p[(int64_t)r * N + i] = i < nv ? floordiv_pos(shl64(lut_exp(T, mx, row[i]), 20), es) : 0;
 }
 
 __global__ void k_embed(const int32_t* __restrict__ ids, const int32_t* __restrict__ emb, int64_t* __restrict__ x,

@@ -110,14 +110,15 @@ __device__ __forceinline__ int64_t isqrt64(int64_t n) {
   return r;
 }
 
-// exp LUT (Q24), d >= 0 for valid entries: e = T[i] - shr((T[i] - T[i+1]) * fr, 8)
-__device__ __forceinline__ int64_t lut_exp(const int32_t* T, int64_t d) {
-  int64_t i = d >> 8;
-  if (i > EXACT_EXP_N - 2) i = EXACT_EXP_N - 2;
-  int64_t fr = d & 255;
-  int64_t a = T[i], b = T[i + 1];
-  int64_t e = a - shr64((a - b) * fr, 8);
-  return d < (40LL << EXACT_F) ? e : 0;
+// exp LUT (Q24) of the distance mx - x of an x <= mx: e = T[i] - shr((T[i] - T[i+1]) * fr, 8), 0 from 40 on. The difference modulo
+// 2^64 is taken as unsigned, which is the distance of any two int64: scores that left int64 can lie 2^63 apart or more.
+__device__ __forceinline__ int64_t lut_exp(const int32_t* T, int64_t mx, int64_t x) {
+  const uint64_t d = (uint64_t)mx - (uint64_t)x;
+  const bool far = d >= (40ULL << EXACT_F);
+  const uint32_t i = far ? EXACT_EXP_N - 2 : (uint32_t)d >> 8;
+  const int64_t fr = d & 255, a = T[i], b = T[i + 1];
+  const int64_t e = a - shr64((a - b) * fr, 8);
+  return far ? 0 : e;
 }
 
 // SiLU (identity above 16) / sigmoid (1.0 above 16) tables on [-16, 16) at 1/256 steps

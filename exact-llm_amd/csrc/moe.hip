@@ -42,9 +42,9 @@ __global__ void k_router_topk(int64_t* __restrict__ t, int ld, const int32_t* __
   }
   mx = block_max64(mx, red);
   int64_t es = 0;
-  for (int i = threadIdx.x; i < NE; i += blockDim.x) es += lut_exp(T, mx - sp[i]);
+  for (int i = threadIdx.x; i < NE; i += blockDim.x) es += lut_exp(T, mx, sp[i]);
   es = block_sum64(es, red);
-  for (int i = threadIdx.x; i < NE; i += blockDim.x) sp[i] = floordiv_pos(shl64(lut_exp(T, mx - sp[i]), 20), es);
+  for (int i = threadIdx.x; i < NE; i += blockDim.x) sp[i] = floordiv_pos(shl64(lut_exp(T, mx, sp[i]), 20), es);
   __syncthreads();
   for (int i = threadIdx.x; i < NE; i += blockDim.x) {
     const int64_t pi = sp[i];
@@ -77,7 +77,7 @@ __device__ __forceinline__ int route_row_w(int64_t* __restrict__ t, int ld, cons
   const int64_t y = in ? shr64(tr[in ? lane : 0], sh) : INT64_MIN;
   if (in && clear_t) tr[lane] = 0;
   const int64_t mx = wave_max64(y);
-  const int64_t e = in ? lut_exp(T, mx - y) : 0;
+  const int64_t e = in ? lut_exp(T, mx, y) : 0;
   const int64_t es = wave_sum64(e);
   const int64_t p = in ? floordiv_pos(shl64(e, 20), es) : -1;   // probabilities are >= 0: lanes past NE rank last
   int rank = 0;

@@ -40,11 +40,11 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void k_sample(const int64_t* __rest
   mx = block_max64(mx, red_a);
   // pass 2: the softmax denominator
   int64_t es = 0;
-  for (int i = b0 + lane; i < b1; i += 64) es += lut_exp(T, mx - shr64(row[i] * tnum, EXACT_F));
+  for (int i = b0 + lane; i < b1; i += 64) es += lut_exp(T, mx, shr64(row[i] * tnum, EXACT_F));
   es = block_sum64(es, red_b);
   // pass 3: each wave's sum of p
   int64_t ps = 0;
-  for (int i = b0 + lane; i < b1; i += 64) ps += floordiv_pos(shl64(lut_exp(T, mx - shr64(row[i] * tnum, EXACT_F)), 20), es);
+  for (int i = b0 + lane; i < b1; i += 64) ps += floordiv_pos(shl64(lut_exp(T, mx, shr64(row[i] * tnum, EXACT_F)), 20), es);
   ps = wave_sum64(ps);
   if (lane == 0) wsum[w] = ps;
   __syncthreads();
@@ -60,7 +60,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void k_sample(const int64_t* __rest
   for (int base = b0; base < b1; base += 64) {
     const int i = base + lane;
     int64_t p = 0;
-    if (i < b1) p = floordiv_pos(shl64(lut_exp(T, mx - shr64(row[i] * tnum, EXACT_F)), 20), es);
+    if (i < b1) p = floordiv_pos(shl64(lut_exp(T, mx, shr64(row[i] * tnum, EXACT_F)), 20), es);
     if (p_out && i < b1) p_out[(int64_t)r * V + i] = p;
     const int64_t c = carry + wave_incl_scan64(p, lane);
     if (i < b1 && c <= target) ++cnt;
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(SAMPLE_NT) void k_sample_exp(const int64_t* __restr
 #pragma unroll
   for (int k = 0; k < SAMPLE_PT; ++k)
     if (B.ok[k]) {
-      const int64_t e = lut_exp(T, mx - a[k]);
+      const int64_t e = lut_exp(T, mx, a[k]);
       wk.e[B.r * V + B.i0 + 64 * k] = (int32_t)e;
       if (e < 0) wk.neg[B.r] = 1;
       es += e;

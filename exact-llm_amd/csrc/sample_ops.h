@@ -13,13 +13,7 @@ __device__ __forceinline__ int64_t wave_incl_scan64(int64_t v, int lane) {
   return v;
 }
 
-// exp LUT of mx - x for x <= mx, however far below
-__device__ __forceinline__ int64_t lut_exp_below(const int32_t* T, int64_t mx, int64_t x) {
-  const uint64_t d = (uint64_t)mx - (uint64_t)x;
-  return d < (40ULL << EXACT_F) ? lut_exp(T, (int64_t)d) : 0;
-}
-
-// The same in 32 bits for a distance d kept against the maximum of a part (at most EXP_FAR, from where exponentials are 0, or EXP_UNSEEN
+// lut_exp in 32 bits for a distance d kept against the maximum of a part (at most EXP_FAR, from where exponentials are 0, or EXP_UNSEEN
 // for a value left out), where that maximum lies gap (exp_gap) below the row's. The last table entries read are 10240 and 10241, and
 // a - shr((a - b) fr, 8) lies between a and b.
 #define EXP_FAR (40U << EXACT_F)

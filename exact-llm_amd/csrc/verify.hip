@@ -292,7 +292,7 @@ __global__ __launch_bounds__(NT) void k_verify_row(VerifyArgs A, VerifyShort W) 
   int32_t e[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    e[k] = j0 + 64 * k < A.V ? (int32_t)lut_exp_below(A.T, m, a[k]) : 0;
+    e[k] = j0 + 64 * k < A.V ? (int32_t)lut_exp(A.T, m, a[k]) : 0;
     if (j0 + 64 * k < A.V) W.e[r * A.V + j0 + 64 * k] = e[k];
     es += e[k];
   }
