@@ -31,10 +31,14 @@ __device__ __forceinline__ int32_t lut_exp_kept(const int32_t* T, uint32_t gap, 
 
 // floor(e 2^20 / es) for e below 2^31 and es < 2^51, at least 0: with es20 = max(es, 1) 2^-20 and rb = (1 - 2^-45) / es20 the estimate
 // is p or p - 1, and its remainder, exact in one fma, tells which. e <= es gives at most 2^20; more (of an exp table with negative
-// entries, whose sum may be small) goes through the division.
+// entries, whose sum may be small) goes through the division and counts as PROB_NONE from there on.
+//
+// A row whose p sum to PROB_NONE or more counts as one without probability (p = 0): below it the products of judging, u q P, p Q 2^20 and
+// u W, stay under 2^63. Only tables with negative entries give sums above 2^20.
+#define PROB_NONE (1LL << 23)
 __device__ __forceinline__ int64_t prob20(int32_t e, int64_t es, double es20, double rb) {
   if (e <= 0 || es <= 0) return 0;
-  if (e > es) return floordiv_pos(shl64(e, 20), es);
+  if (e > es) return min(floordiv_pos(shl64(e, 20), es), PROB_NONE);   // so that 2^30 of them sum up in 64 bits
   const double p = __builtin_floor((double)e * rb);
   return (int64_t)(uint32_t)p + (__builtin_fma(-p, es20, (double)e) >= es20);
 }

@@ -2,7 +2,8 @@
 //   p = isoftmax_row(shr(lg * tnum, 16)) (Q20), P = sum p; q (Q20) the draft model's probabilities, Q = sum q
 // A token x drafted from q is accepted with probability min(1, (p / P) / (q / Q)): u q(x) P < p(x) Q 2^20 for a u of [0, 2^20).
 // After a rejection the token comes from w = max(p Q - q P, 0), which together make the tokens distributed as p / P. Every
-// product is below 2^60 (p, q, P, Q <= 2^20), so both are exact in int64.
+// product is below 2^60 (p, q, P, Q <= 2^20), so both are exact in int64; with an exp table with negative entries below 2^63, since a row
+// whose p sum to 2^23 or more counts as one without probability.
 #include "exact_common.h"
 #include "abi_util.h"
 #include "sample_ops.h"
@@ -167,7 +168,8 @@ __global__ __launch_bounds__(VERIFY_NT) void k_verify_rest(VerifyArgs A, VerifyW
     const int64_t qx = in ? A.q[((int64_t)b * A.K + i) * A.V + x] : 0;
     const int32_t ex = in ? (int32_t)W.d[r * A.V + x] : 0;
     const int u = A.u[r];
-    const RowSums R = row_sums(W, r, nch, lane);
+    RowSums R = row_sums(W, r, nch, lane);
+    if (R.P >= PROB_NONE) R.es = R.P = 0;
     const double es20 = sum20(R.es);
     if (lane == 0) {
       rows[i] = R;
@@ -237,6 +239,7 @@ __global__ __launch_bounds__(VERIFY_NT) void k_verify_pick(VerifyArgs A, VerifyW
   int64_t total = a < A.count(b) ? wave_total(sums, nch, lane) : 0;
   const bool rest = total > 0;
   if (!rest) sums = W.ps + r * nch, total = P;
+  if (total == 0) return;
   int64_t carry = wave_total(sums, c, lane);
   const int64_t target = verify_target(A.u[r0 + A.K], total);
   if (target < carry || target >= carry + sums[c]) return;
@@ -310,11 +313,12 @@ __global__ __launch_bounds__(NT) void k_verify_row(VerifyArgs A, VerifyShort W) 
   __syncthreads();
   if (threadIdx.x) return;
   for (int w = 1; w < NT / 64; ++w) P += red[2][w], Q += red[3][w];
+  const bool none = P >= PROB_NONE;
   int64_t* at = W.at + 4 * r;
-  at[0] = es;
-  at[1] = P;
+  at[0] = none ? 0 : es;
+  at[1] = none ? 0 : P;
   at[2] = Q;
-  at[3] = in && verify_accepts(u, px, P, qx, Q);
+  at[3] = in && !none && verify_accepts(u, px, P, qx, Q);
 }
 
 // grid B: the first row whose token is rejected (or the one after the last token), the rest's weights there and the token picked by them

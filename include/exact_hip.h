@@ -511,7 +511,8 @@ int exact_sample_split(const int64_t* lg, int32_t R, int32_t V, uint64_t seed, c
 /* Drafted tokens of a draft model judged against the target's logits (speculative sampling), in the sampler's integers. Sequence b
  * drafted tok[b K .. ), drafted[b] <= K of them (NULL: K); lg (B, K + 1, V): the target's logits before each drafted token and after
  * the last; q (B, K, V): the draft's probabilities as exact_sample's p_out gives them (not negative, a row's sum Q at most 2^20). With
- * p = isoftmax_row(rs(lg * tnum, 16)) (a negative p counts as 0) and P = sum p, token x is accepted if u q(x) P < p(x) Q 2^20, where
+ * p = isoftmax_row(rs(lg * tnum, 16)) and P = sum p (with an exp table with negative entries: a negative p counts as 0, and a row whose
+ * exponentials sum to 0 or less, or whose P is 2^23 or more, as one of p = 0), token x is accepted if u q(x) P < p(x) Q 2^20, where
  * u (B, K + 1) holds random numbers (their low 20 bits are taken): with probability min(1, (p / P) / (q / Q)). The first row a whose
  * token is not (a token outside the vocabulary never is) gives the token that follows from w = max(p Q - q P, 0) (from p where all of w
  * is 0), the row after the last token from w = p: #{j : w_0 + .. + w_j <= (u[b][K] sum w) >> 20}, V where all of p is 0. ids (B, K + 1):

@@ -570,11 +570,23 @@ def tree_attention(t, s, b, cos, sin, slot, base, depth, mask, nodes, cache, H, 
     return out.reshape(B * T, H * hd)
 
 
-def verify_draft(lg, q, tok, u, tnum, drafted):
+def judged_row(sc, table=None):
+    """p of a target row as judging takes it (Python integers): isoftmax_row's; of a table with negative entries no p below 0, and none at
+    all where the exponentials sum to 0 or less or p to 2^23 or more."""
+    T = EXP_T if table is None else np.asarray(table, I64)
+    d = sc.max() - sc
+    i = np.minimum(d >> I64(EXP_STEP), len(T) - 2)
+    e = np.where(d < (40 << F), T[i] - round_shift((T[i] - T[i + 1]) * (d & I64((1 << EXP_STEP) - 1)), EXP_STEP), 0)
+    es = int(e.sum())
+    p = [max((int(x) << 20) // es, 0) for x in e] if es > 0 else [0] * len(e)
+    return p if sum(p) < 1 << 23 else [0] * len(p)
+
+
+def verify_draft(lg, q, tok, u, tnum, drafted, table=None):
     """One sequence's drafted tokens judged (Python integers): (accepted tokens + the one that follows, how many were accepted)."""
     got, K = [], len(tok)
     for i in range(drafted + 1):
-        p = [max(int(x), 0) for x in isoftmax_row(round_shift(np.asarray(lg[i], I64) * tnum, 16))]
+        p = judged_row(round_shift(np.asarray(lg[i], I64) * tnum, 16), table)
         P, w = sum(p), p
         if i < drafted:
             qi, x = [int(a) for a in q[i]], int(tok[i])

@@ -115,3 +115,16 @@ def test_tree_accept_takes_the_lowest_matching_child():
     assert O.tree_accept([7, 8, 8, 9], [1, 7, 7, 8], [-1, 0, 0, 2], 4) == ([0, 1], [7, 8])
     assert O.tree_accept([7, 8], [1, 7], [-1, 0], 1) == ([0], [7])
     assert O.tree_accept([7], [1], [-1], 0) == ([], [])
+
+
+def test_judged_rows_are_the_samplers_and_their_sums_are_bounded():
+    """the usual table: isoftmax_row's p; tables with negative entries: sums below 2^23 as they are, none from there on"""
+    rng = np.random.default_rng(6)
+    sc = rng.integers(-(6 << 16), 6 << 16, 300)
+    assert O.judged_row(sc) == O.isoftmax_row(sc).tolist()
+    T = np.full(10242, -(1 << 14))
+    T[0] = 1 << 24   # the row's largest gives 2^24, every other one within 40 takes 2^14 off
+    for near, P in ((0, 1 << 20), (512, 1 << 21), (895, (1 << 30) // 129), (896, 0), (1023, 0), (1024, 0), (1500, 0)):
+        row = np.full(2000, -(50 << 16))
+        row[7], row[100:100 + near] = 0, -(1 << 16)
+        assert sum(O.judged_row(row, T)) == P
