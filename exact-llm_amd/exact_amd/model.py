@@ -1121,7 +1121,9 @@ class TreeDecoder:
     """Decoding by passes over drafted token trees, B sequences (slots 0 .. B - 1 of the cache) of up to T <= 64 nodes. Node 0 is a
     sequence's last token, whose key is not in the cache yet; the others may follow it. One pass gives every node's logits
     and the target's token after it (greedy, or sampled with seed and temp by the node's own step); the path along which the tree
-    holds those very tokens is kept in the cache, so the tokens are exactly those of decoding one at a time."""
+    holds those very tokens is kept in the cache, so the tokens are exactly those of decoding one at a time. The seed is one for all
+    sequences and a random number belongs to its step alone: sequences that have to differ (slots forked from one prompt) take
+    steps apart, such as from b << 20 on."""
 
     def __init__(self, tm, cache, B, T, seed=None, temp=1.0):
         if not 1 <= T <= ops.TREE_MAX or not 1 <= B <= cache.B:
@@ -1207,7 +1209,7 @@ class TreeDecoder:
 
     def step(self, tokens, parents, steps=None):
         """One pass: tokens[b] and parents[b] are sequence b's tree (parents -1 for node 0), steps[b] the sampler's step of the token
-        after node 0. Returns (new tokens of each sequence: the accepted ones and the one that follows them, their
+        after node 0 (needed with a seed). Returns (new tokens of each sequence: the accepted ones and the one that follows them, their
         paths: the nodes whose logits gave them); the cache then holds all but the last of the new tokens."""
         self.start(tokens, parents, steps)
         return self.finish()
@@ -1216,6 +1218,8 @@ class TreeDecoder:
         """step()'s pass, left running on the current stream; finish() waits for it."""
         if self.running:
             raise ExactError("the pass before has to be finished first")
+        if steps is None and self.seed is not None:
+            raise ExactError("sampled trees need the step of each sequence's next token")
         self._load(tokens, parents, [0] * self.B if steps is None else steps)
         if self.graphs is None:
             self.tree.keys = min(self.cache.Smax, max(self.cache.n[:self.B]) + self.T)

@@ -1,5 +1,6 @@
 """The model's paths over drafted tokens: trees, a draft model, forked sequences. Drafts change how many tokens a pass gives, never
 which, so receipts, tokens, logits and cache rows are compared with decoding one token at a time."""
+import os
 import random
 
 import numpy as np
@@ -277,3 +278,53 @@ def test_lookup_draft_shares_prefixes():
     assert lookup_draft([1, 2, 3, 4, 1, 2, 5, 6, 1, 2]) == ([5, 6, 1, 2, 3, 4, 1, 2, 5], [-1, 0, 1, 2, -1, 4, 5, 6, 7])
     assert lookup_draft([1, 2, 3, 9, 1, 2, 3, 8, 1, 2], length=2) == ([3, 8, 9], [-1, 0, 0])
     assert lookup_draft([1]) == lookup_draft([1, 2, 3]) == ([], [])
+
+
+def sampled(tm, prompt, n, seed, temp, step0):
+    """n sampled tokens one at a time, the sampler's steps from step0 on"""
+    cache, ids, toks = tm.new_cache(B=1), torch.zeros(1, dtype=torch.int32, device=DEV), []
+    lg = tm.forward(prompt, cache, last_only=True)
+    for i in range(n):
+        ops.sample(lg, seed, torch.full((1,), step0 + i, dtype=torch.int32, device=DEV), ops.temp_num(temp), tm.tab.exp, ids)
+        toks.append(int(ids))
+        lg, _ = tm.decode_rows(toks[-1:], cache)
+    return toks
+
+
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("first", [(0, 0, 5), (0, 1 << 20, 0)])
+def test_seeded_trees_of_a_batch(graph, first):
+    """one seed for a forked prompt's two slots and another prompt's: the tokens of sampling one at a time at each sequence's own
+    steps, so that equal steps continue the fork alike and steps apart differ"""
+    tm, seed, temp = model("tiny-hd128", batch=3), 9, 1.2
+    prompts = [helpers.prompt(1, 11, tm.cfg.V)] * 2 + [helpers.prompt(2, 6, tm.cfg.V)]
+    true = [sampled(tm, p, 14, seed, temp, f) for p, f in zip(prompts, first)]
+    assert (true[0] == true[1]) == (first[0] == first[1])
+    cache = tm.new_cache()
+    tm.forward(prompts[0], cache, last_only=True, slot=0)
+    cache.fork(0, [1])
+    tm.forward(prompts[2], cache, last_only=True, slot=2)
+    td = TreeDecoder(tm, cache, 3, 7, seed=seed, temp=temp)
+    if graph:
+        td.capture()
+    out = [t[:1] for t in true]
+    for it in range(3):
+        drafts = [guesses(true[b], it + b, 0.8)(out[b]) for b in range(3)]
+        new, _ = td.step([[o[-1]] + t[:6] for o, (t, _) in zip(out, drafts)], [[-1] + [x + 1 for x in p[:6]] for _, p in drafts],
+                         [f + len(o) for f, o in zip(first, out)])
+        for b in range(3):
+            out[b] += new[b]
+            assert out[b][:14] == true[b][:len(out[b])]
+
+
+def test_seeded_steps_have_to_be_given():
+    """every pass would draw the random numbers of step 0 again"""
+    tm = model("tiny", Smax=32)
+    cache = tm.new_cache()
+    tm.forward([1, 2, 3], cache, last_only=True)
+    td = TreeDecoder(tm, cache, 1, 4, seed=5)
+    for call in (td.step, td.start):
+        with pytest.raises(ops.ExactError):
+            call([[1]], [[-1]])
+    assert cache.n[0] == 3 and len(td.step([[1]], [[-1]], [1])[0][0]) == 1 and cache.n[0] == 4
+    assert len(TreeDecoder(tm, cache, 1, 4).step([[1]], [[-1]])[0][0]) == 1   # greedy ones take no steps
