@@ -1139,7 +1139,7 @@ class TreeDecoder:
         self.ws.next_ids = z(B * T)   # beside the input ids, which tree_accept compares them with
         self.path, self.ids, self.n = z(B, T), z(B, T), z(B)
         self.graphs = None   # bound of the positions -> captured pass
-        self.running = False
+        self.running, self.stream = False, None   # a pass was started, on that stream
 
     def _load(self, tokens, parents, steps):
         B, T, n = self.B, self.T, self.cache.n
@@ -1215,7 +1215,7 @@ class TreeDecoder:
         return self.finish()
 
     def start(self, tokens, parents, steps=None):
-        """step()'s pass, left running on the current stream; finish() waits for it."""
+        """step()'s pass, left running on the current stream; finish() waits for it, whichever stream is current then."""
         if self.running:
             raise ExactError("the pass before has to be finished first")
         if steps is None and self.seed is not None:
@@ -1226,14 +1226,15 @@ class TreeDecoder:
             self._pass()
         else:
             self._captured().replay()
-        self.running = True
+        self.running, self.stream = True, torch.cuda.current_stream()
 
     def finish(self):
         """What step() returns, of the pass that was started."""
         if not self.running:
             raise ExactError("no pass was started")
         self.running = False
-        got = torch.cat([self.n[:, None], self.ids, self.path], 1).tolist()
+        with torch.cuda.stream(self.stream):
+            got = torch.cat([self.n[:, None], self.ids, self.path], 1).tolist()
         out = [(r[1:1 + r[0]], r[1 + self.T:1 + self.T + r[0]]) for r in got]
         for b, (ids, _) in enumerate(out):
             self.cache.n[b] += len(ids)

@@ -328,3 +328,34 @@ def test_seeded_steps_have_to_be_given():
             call([[1]], [[-1]])
     assert cache.n[0] == 3 and len(td.step([[1]], [[-1]], [1])[0][0]) == 1 and cache.n[0] == 4
     assert len(TreeDecoder(tm, cache, 1, 4).step([[1]], [[-1]])[0][0]) == 1   # greedy ones take no steps
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_a_pass_started_on_another_stream(graph):
+    """finish() waits for the pass, whichever stream is current then"""
+    tm = model("tiny")
+    caches = [tm.new_cache(), tm.new_cache()]
+    tds = []
+    for c in caches:
+        tm.forward([5, 6, 7, 8], c, last_only=True)
+        tds.append(TreeDecoder(tm, c, 1, 4))
+        if graph:
+            tds[-1].capture()
+    td, ref = tds
+    tree = [[9, 3, 4, 5]], [[-1, 0, 0, 1]]
+    want = ref.step(*tree)
+    x = torch.randn((8192, 8192), dtype=torch.bfloat16, device=DEV)
+    side, load = torch.cuda.Stream(), td._load
+
+    def busy(*a):   # the pass lies behind some 50 ms of other work
+        load(*a)
+        for _ in range(50):
+            x @ x
+
+    td._load = busy
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        td.start(*tree)
+    assert td.finish() == want
+    lg = td.logits_rows(0, want[1][0])
+    assert torch.equal(lg, ref.logits_rows(0, want[1][0]))
