@@ -359,3 +359,39 @@ def test_a_pass_started_on_another_stream(graph):
     assert td.finish() == want
     lg = td.logits_rows(0, want[1][0])
     assert torch.equal(lg, ref.logits_rows(0, want[1][0]))
+
+
+def test_trees_of_a_per_channel_model():
+    """separate q, k, v linears with one scale a channel: receipts and logits of plain decoding"""
+    z = np.load(os.path.join(os.path.dirname(__file__), "golden", "intmodel_tiny.npz"))
+    cfg = synth.ModelConfig("channel", D=128, H=2, KV=1, hd=64, I=256, V=512, NL=2, theta=10000.0)
+    arrays = {k: z[k] for k in z.files}
+    arrays["emb"] = z["emb"].astype(np.int64)
+    tm = TModel(DeviceWeights.from_arrays(cfg, arrays, DEV, mode="channel"), Smax=64)
+    prompt = helpers.prompt(4, 8, cfg.V)
+    want, greedy = generate(tm, prompt, 30, 2, 0.9)
+    for nodes, good in ((1, 1.0), (4, 0.8), (20, 1.0), (40, 0.5)):
+        got, g = generate(tm, prompt, 30, 2, 0.9, draft=guesses(prompt + want["tokens"], nodes, good), nodes=nodes)
+        assert got == want and g == greedy, nodes
+
+
+def test_captured_trees_with_eager_passes_between():
+    """prompts, decode steps and other trees of the same model, run eagerly on another cache between the replays"""
+    tm = model("tiny-moe")
+    prompt = helpers.prompt(6, 10, tm.cfg.V)
+    want, _ = generate(tm, prompt, 16, 8, 1.0)
+    cache, other = tm.new_cache(), tm.new_cache()
+    tm.forward(prompt, cache, last_only=True)
+    td = TreeDecoder(tm, cache, 1, 8, seed=8, temp=1.0)
+    td.capture()
+    out, it = want["tokens"][:1], 0
+    while len(out) < 12:
+        t, p = guesses(prompt + want["tokens"], it, 0.8)(prompt + out)
+        (new,), _ = td.step([[out[-1]] + t[:7]], [[-1] + [x + 1 for x in p[:7]]], [len(out)])
+        out += new
+        assert out[:16] == want["tokens"][:len(out)]
+        other.n[0] = 0
+        tm.forward(helpers.prompt(it, 20 + it, tm.cfg.V), other, last_only=True)
+        tm.decode_rows([3], other)
+        TreeDecoder(tm, other, 1, 5).step([[1, 2, 3]], [[-1, 0, 0]])
+        it += 1
