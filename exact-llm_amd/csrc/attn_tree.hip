@@ -2,7 +2,8 @@
 // exact_llm.py:164-176 for rows of which each sees the cached positions and the nodes its mask names.
 //
 // A tree's nodes lie behind the cached positions, node i at base + i, while RoPE turns a node by its depth, so the key of an
-// accepted node is right wherever it is moved to afterwards.
+// accepted node is right wherever it is moved to afterwards. Rows of padding nodes are computed as the others are, over all keys,
+// and come out as zeros.
 #include "exact_common.h"
 #include "abi_util.h"
 #include "sample_ops.h"
@@ -71,7 +72,7 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& A, int b) {
 
 // grid (B T, H + 2 KV), one wave a head: y = shr(t, 28 - s) + b, RoPE at base + depth, qrow; query digits to the workspace, key and
 // value to the cache at base + node. Queries of dead nodes are zeros. Latency: 3.6 us for 8 rows of 18 heads of 64, 12.5 us for 256 rows of
-// 56 heads of 128 (36 MB read and written).
+// 56 heads of 128 (20 MB read and written; clear_t writes 15 more).
 template <int HD>
 __global__ __launch_bounds__(64) void k_tree_qkv(int64_t* __restrict__ t, const int32_t* __restrict__ s,
                                                  const int64_t* __restrict__ b, const int64_t* __restrict__ cos_t,
@@ -321,9 +322,10 @@ __device__ __forceinline__ void byte_planes(const uint32_t* a, int& b0, int& b1,
 // grid (M, KV, B), one block a row: its maximum from the groups', the exponentials, their sum, and p as its three balanced base-256
 // digits over the distances (p is made as prob20 makes it, whose conditions hold where no exponential is negative); clears the p.V
 // totals. The first distances are in flight while the maximum is found and their exponentials stay in registers; those of longer rows
-// are made again. A quad of keys lies within the lane's own 128 keys, which one wave reads before it writes them. Bound by the bytes:
-// 105 us for 62 million distances, 7 read and written each, 4.1 TB/s. Seven waves a SIMD are asked for, because with all the registers
-// every table entry of the row is loaded ahead and few waves are left (332 us).
+// are made again. A quad of keys lies within the lane's own 128 keys, which one wave reads before it writes them. Bound by about 40
+// vector instructions a distance, which keep the SIMDs 73% busy: 105 us for 62 million distances, 7 bytes read and written each (4.1 TB/s;
+// with distances and digits in 24 bits, a quarter less, the launch took 95 and the value product as much more). Seven waves a SIMD are
+// asked for, because with all the registers every table entry of the row is loaded ahead and few waves are left (332 us).
 template <int HD>
 __global__ __launch_bounds__(256, 7) void k_tree_exp(const int32_t* __restrict__ expt, TreeArgs A, TreeWork W) {
   __shared__ int64_t red[2][16];
@@ -897,6 +899,8 @@ static int64_t tree_work(const TreeArgs& A, int hd, int8_t* at, TreeWork& W) {
 // the totals' atomics 8 ns each; the cheapest of all numbers of tiles and of up to four rounds of blocks (256 CUs) is taken. us a layer, 28
 // heads over 4 of 128 at 1793 positions, a tree of 26: 1 tile in 5 runs (taken) 36.3, 2 in 10 36.0, 3 in 8 37.0, 3 in 15 37.8; 40 over 8 at
 // 6001, four trees of 64: 5 tiles in 2 runs (taken) 321, 3 in 5 394, 2 in 5 463, 1 in 5 569.
+// Heads of 64 have no term of their own: 14 over 2, four trees of 64 at 6001: 5 tiles in 5 runs (taken) 107, 3 in 3 108, 2 in 2 115, 1 in
+// 1 140; a tree of 26 at 1793: 2 in 15 (taken) 28.3, 2 in 8 26.3, 1 in 8 25.6.
 struct TreeSplit {
   int mt, groups, ksplit;
 };

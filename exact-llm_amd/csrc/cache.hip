@@ -6,14 +6,17 @@
 namespace exact {
 
 #define CACHE_NT 256
-#define CACHE_ROWS 8   // rows in flight in k_cache_keep: 8 paths in 48 layers of 8 heads of 128 take 11.2 us, with 4 11.5, with 16 17.1 (registers)
+// rows in flight in k_cache_keep. us for 8 paths of 6, 16 and 56 nodes in 48 layers of 8 heads of 128 with 4 / 8 / 16: 12.8 / 12.6 / 19.4,
+// 29.1 / 28.6 / 40.2, 139 / 137 / 187 (registers)
+#define CACHE_ROWS 8
 #define CACHE_CK 64    // positions a block of k_cache_fork
 
 // grid (units of a position, B, L): a thread owns 16 bytes (or the shift) of one (layer, sequence, KV head)'s rows and moves them from base
 // + path[d] to base + d for d = 0, 1, ... An accepted path goes up, so path[d] >= d: a row is read before any row that is written over it,
 // and the first CACHE_ROWS rows can be loaded together. A path that does not go up ends there. A sequence whose slot one before it has
-// would race: it is left out. Latency of the rounds of CACHE_ROWS rows: 3.5 us for 24 layers of 2 heads of 64, 11.2 us for 8 paths of up to
-// 64 in 48 layers of 8 heads of 128.
+// would race: it is left out. Latency of the loads of slots, counts and path, one after the other behind a barrier, and of the rounds of
+// CACHE_ROWS rows, up to near the copy rate where many rows move. us in a graph: one path of 1 / 8 / 56 rows in 24 layers of 2 heads of 64
+// 4.6 / 7.5 / 38, 8 paths of 1 / 6 / 16 / 56 in 48 layers of 8 heads of 128 5.8 / 12.6 / 28.6 (4.1 TB/s) / 137 (3.2 TB/s).
 __global__ __launch_bounds__(CACHE_NT) void k_cache_keep(v4i* __restrict__ kq, int32_t* __restrict__ sk, v4i* __restrict__ v,
                                                          int nslots, const int32_t* __restrict__ slot,
                                                          const int32_t* __restrict__ base, const int32_t* __restrict__ path,
@@ -57,7 +60,8 @@ __global__ __launch_bounds__(CACHE_NT) void k_cache_keep(v4i* __restrict__ kq, i
 
 // grid (chunks of CACHE_CK positions, L KV, pairs): the chunk's rows of one (layer, KV head) from slot src to slot dst, which are
 // contiguous in each array. A pair whose dst is a source, or the dst of a pair before it, is left out: it would race. Copy rate: 301 us,
-// 5.1 TB/s, for 1793 positions of 28 layers of 4 heads of 128 to three slots; 7.2 us for 137 positions of 24 layers of 2 heads of 64.
+// 5.1 TB/s, for 1793 positions of 28 layers of 4 heads of 128 to three slots; 7.2 us for 137 positions of 24 layers of 2 heads of 64, whose
+// 144 blocks leave 112 CUs idle.
 __global__ __launch_bounds__(CACHE_NT) void k_cache_fork(v4i* __restrict__ kq, int32_t* __restrict__ sk, v4i* __restrict__ v,
                                                          int nslots, const int32_t* __restrict__ src,
                                                          const int32_t* __restrict__ dst, const int32_t* __restrict__ n, int M,

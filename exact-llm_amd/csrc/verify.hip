@@ -17,7 +17,8 @@ namespace exact {
 // owns PT * 64 consecutive logits. One block walks a row of 151936 logits four times in 190 us; a launch here starts from the
 // chunk results of the one before. The logits are read once: the first launch keeps them as 32-bit distances to their chunk's maximum,
 // the second as exponentials, which every later launch reads (74.4 us for 8 sequences of 7 drafts at 152064; made again by each, 78.6).
-// The first launch reads 14.5 bytes a logit at 5.6 TB/s, the others 4 that the caches hold in part.
+// The first launch of that call reads 129 MB of logits and q at 4.85 TB/s (6.15 with the distances that it writes), the others 4 bytes a
+// logit that the caches hold in part.
 #define VERIFY_NT 256
 // logits of a row that one block holds: with 8000, one row takes 19.4 us (over chunks 17.0), 9 rows 20.8 (22.3), 160 rows 22.0 (25.1)
 #define VERIFY_SHORT 8192
@@ -34,7 +35,7 @@ struct VerifyArgs {
 struct VerifyWork {
   int64_t *mx, *es, *ps, *qs;   // [B (K + 1)][nch]: of each chunk the maximum, sums of exponentials, of p and of q
   int64_t* ws;                  // [B][nch]: sum of the rest's weights in the row that rejected
-  int64_t* at;                  // [B][5]: that row (or the one after the last token), its maximum, sum of exponentials, P, Q
+  int64_t* at;                  // [B][4]: that row (or the one after the last token), its sum of exponentials, P, Q
   uint32_t* d;                  // [B (K + 1)][V]: maximum of the chunk - logit, then exponentials
 };
 

@@ -949,7 +949,9 @@ def speculate(tm, dm, prompt_ids, n, seed, temp, k=4):
     cache, dcache = tm.new_cache(B=1), dm.new_cache(B=1)
     z = lambda *sh, dt=I32: torch.zeros(sh, dtype=dt, device=dev)
     q, tok, ids, acc, step, one = z(1, k, V, dt=I64), z(1, k), z(1, k + 1), z(1), z(1), z(1)
-    dkey, jkey = synth.key(seed, "draft"), synth.key(seed, "judge")   # every draw has a random number of its own
+    dkey, jkey = synth.key(seed, "draft"), synth.key(seed, "judge")
+    # judging has random numbers of its own; a draft's belongs to its position, so those of the drafts behind a rejected one come again
+    # in the next pass: no kept token depends on them
     ops.sample(tm.forward(prompt, cache, last_only=True), seed, step, tnum, tm.tab.exp, one)
     toks, counts = one.tolist(), []
     while len(toks) < n:
