@@ -35,10 +35,13 @@ __device__ __forceinline__ int32_t lut_exp_kept(const int32_t* T, uint32_t gap, 
 //
 // A row whose p sum to PROB_NONE or more counts as one without probability (p = 0): below it the products of judging, u q P, p Q 2^20 and
 // u W, stay under 2^63. Only tables with negative entries give sums above 2^20.
-#define PROB_NONE (1LL << 23)
+#define PROB_NONE ((int64_t)1 << 23)
 __device__ __forceinline__ int64_t prob20(int32_t e, int64_t es, double es20, double rb) {
   if (e <= 0 || es <= 0) return 0;
-  if (e > es) return min(floordiv_pos(shl64(e, 20), es), PROB_NONE);   // so that 2^30 of them sum up in 64 bits
+  if (e > es) {
+    const int64_t p = floordiv_pos(shl64(e, 20), es);
+    return p < PROB_NONE ? p : PROB_NONE;   // 2^30 of them sum up in 64 bits
+  }
   const double p = __builtin_floor((double)e * rb);
   return (int64_t)(uint32_t)p + (__builtin_fma(-p, es20, (double)e) >= es20);
 }
