@@ -835,6 +835,8 @@ def generate(tm, prompt_ids, n, seed, temp, draft=None, nodes=16):
     tree, -1 for the last token so far), as lookup_draft() does; up to nodes rows are then judged a pass, with the same
     receipt, since every accepted token is the one that its own logits row and step sample.
     Returns (receipt dict, greedy tokens)."""
+    if n < 1:
+        return dict(prompt=list(prompt_ids), seed=seed, temp=temp, tokens=[], chain="start"), []
     if draft is not None:
         return _generate_drafted(tm, list(prompt_ids), n, seed, temp, draft, nodes)
     tnum = ops.temp_num(temp)

@@ -183,3 +183,13 @@ def test_no_rows_are_refused(V):
     z = lambda *sh, dt=I32: torch.zeros(sh, dtype=dt, device=DEV)
     with pytest.raises(ops.ExactError, match="bad argument"):
         ops.sample(z(0, V, dt=I64), 1, z(0), ops.temp_num(1.0), torch.tensor(exp_t(), dtype=I32, device=DEV), z(0))
+
+
+@pytest.mark.parametrize("draft", [None, lambda tokens: ([], [])])
+def test_generations_of_no_tokens(draft):
+    """an empty receipt, as the oracle's, which verifies"""
+    cfg = synth.CONFIGS["tiny"]
+    tm = TModel(DeviceWeights.synthetic(cfg, 3, DEV), Smax=32)
+    want, greedy, _ = O.generate(helpers.oracle_model(cfg, 3, T=32), [4, 9], 0, seed=1, temp=0.7)
+    got, g = generate(tm, [4, 9], 0, 1, 0.7, draft=draft)
+    assert got == want and g == greedy == [] and verify(tm, got) == (True, None)
